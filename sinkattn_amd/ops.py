@@ -31,10 +31,11 @@ def _require_cuda(name: str, *tensors: torch.Tensor) -> None:
 
 
 def _kernel_operand(t: torch.Tensor) -> torch.Tensor:
-    """Return t if the kernels can address it in place, else a contiguous copy."""
+    """Return t if the kernels can address it in place, else a contiguous copy (a new one: torch calls a tensor
+    contiguous whatever the strides of its dims of size 1 and the alignment of its memory)."""
     s = t.stride()
     ok = len(s) == 4 and s[3] == 1 and not (s[0] | s[1] | s[2]) & 7 and not t.data_ptr() & 15
-    return t if ok else t.contiguous()
+    return t if ok else torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
 
 
 def _pad_head_dim(t: torch.Tensor, to: Optional[int] = None) -> torch.Tensor:
@@ -264,9 +265,12 @@ def _grad_operand(t: torch.Tensor) -> torch.Tensor:
 
 
 def _grad_output(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """An uninitialised gradient of t [B, H, N, D], in t's order of dims where the kernels can write it."""
+    """An uninitialised gradient of t [B, H, N, D], in t's order of dims where the kernels can write it (a dim of size
+    1 may have any stride in t, which empty_like keeps)."""
     out = torch.empty_like(t, dtype=dtype)
-    return out if out.stride(3) == 1 else torch.empty(t.shape, dtype=dtype, device=t.device)
+    s0, s1, s2, s3 = out.stride()
+    ok = s3 == 1 and s2 >= t.shape[3] and not (s0 | s1 | s2) & 7
+    return out if ok else torch.empty(t.shape, dtype=dtype, device=t.device)
 
 
 @functools.lru_cache(maxsize=256)

@@ -1,0 +1,62 @@
+"""Calls of the gradient operators and their autograd forms that a program may make around the usual ones: operands of
+unusual strides, buffers used again, masks that change, streams, other ways of differentiation."""
+import math
+
+import pytest
+import torch
+
+from sinkattn_amd import autograd, ops
+from sinkattn_amd import sparse_attention as sa
+
+from backward_bars import check, formula, make, make_mask, plans
+
+pytestmark = pytest.mark.gpu
+
+
+def odd_view(t, what):
+    """t's values with strides in its dims of size 1, or on an address, that no kernel takes."""
+    B, H, N, D = t.shape
+    if what == "one row":
+        x = torch.empty(B, H, D, 1, dtype=t.dtype, device=t.device).transpose(2, 3)
+    elif what == "one batch":
+        x = torch.empty(H, N, D, 1, dtype=t.dtype, device=t.device).permute(3, 0, 1, 2)
+    else:
+        x = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape)
+    return x.copy_(t)
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 32)])
+@pytest.mark.parametrize("what,B,Nq,Nk", [("one row", 2, 1, 1), ("one batch", 1, 200, 300), ("odd address", 2, 130, 70)])
+def test_odd_strides(dtype, D, what, B, Nq, Nk):
+    """Dims of size 1 with odd strides and odd addresses: the plain layout's results, in the op and through autograd."""
+    ts = make(B, 3, Nq, Nk, D, dtype, layout="bhnd", seed=71)
+    mask = make_mask(B, 3, Nq, Nk, 1.0)
+    plan, kplan = plans(mask)
+    q, k, v, do = ts
+    out, lse = ops.block_sparse_attention(q, k, v, plan)
+    want = ops.block_sparse_attention_backward(do, q, k, v, out, lse, plan, kplan)
+    q, k, v, do, o = (odd_view(t, what) for t in (*ts, out))
+    got = ops.block_sparse_attention_backward(do, q, k, v, o, lse, plan, kplan)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    y, _ = sa._block_sparse_attn(*leaves, mask)
+    assert torch.equal(y, out)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, do), want))
+
+
+@pytest.mark.parametrize("what,B,N", [("one row", 2, 25), ("one batch", 1, 100), ("odd address", 2, 100)])
+def test_pool_odd_strides(what, B, N):
+    """The pooling's gradient from an output gradient of such strides."""
+    gap = 30
+    x = make(B, 2, N, N, 64, torch.bfloat16, layout="bhnd", seed=72)[0]
+    rows = -(-N // gap)
+    d = make(B, 2, rows, rows, 64, torch.bfloat16, layout="bhnd", seed=73)[0]
+    want = ops.mean_pool_tokens_backward(d, N, gap)
+    got = ops.mean_pool_tokens_backward(odd_view(d, what), N, gap, add=None)
+    assert torch.equal(got, want)
+    leaf = x.clone().requires_grad_()
+    y = sa._mean_pool_sequence(leaf, gap)
+    assert torch.equal(torch.autograd.grad(y, leaf, odd_view(d, what))[0], want)
+    if what != "one row":
+        more = odd_view(x, what)
+        assert torch.equal(ops.mean_pool_tokens_backward(d, N, gap, add=more), ops.mean_pool_tokens_backward(d, N, gap, add=x))
