@@ -22,6 +22,15 @@ def needs_grad(*tensors: Optional[torch.Tensor]) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def copy_into(out: torch.Tensor, res: torch.Tensor) -> torch.Tensor:
+    """res copied into `out`, which takes res's place in the graph.  All of `out` is overwritten, so a whole
+    tensor's own history ends here: torch's copy_ keeps it, and a buffer used again would hold every earlier call's
+    graph and run through it.  (Of a view only a part of its base is overwritten: the base's history stays.)"""
+    if out.grad_fn is not None and not out._is_view():
+        out.detach_()
+    return out.copy_(res)
+
+
 def _plans(mask: torch.Tensor) -> Tuple[ops.BlockSparsePlan, ops.BlockSparsePlan]:
     """The mask's plan and key plan.  A capture makes both of its own, from the mask as it is at each replay: a
     cached plan may be freed before the graph, and one made by a graph holds nothing before a replay."""

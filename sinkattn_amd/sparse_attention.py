@@ -683,7 +683,9 @@ def _block_sparse_attn_with_compensation(q: torch.Tensor, k: torch.Tensor, v: to
     one online softmax (fp32 LSEs; the reference rounds both LSEs to q.dtype first).
     Rows at or beyond `compensated_rows` (a multiple of 128) get the sparse part only.
     k_dynamic/v_dynamic must share k's/v's row strides (as ops.mean_pool_kv gives them).
-    Where an input asks for a gradient, `out` gets a copy of the result, with its place in the graph.
+    Where an input asks for a gradient, `out` gets a copy of the result, with its place in the graph.  What
+    a whole tensor held before, an earlier call's result for one, leaves the graph, so a buffer serves call after
+    call; a view is written as by any in-place operation of torch, and its base keeps its history.
     """
     _ensure_block_sparse_available()
     mask = block_mask if block_mask.is_cuda else block_mask.to(q.device)
@@ -691,7 +693,7 @@ def _block_sparse_attn_with_compensation(q: torch.Tensor, k: torch.Tensor, v: to
         if out is not None:
             ops._check_output(out, q)
         res = autograd.block_sparse_attention_comp(q, k, v, mask, k_dynamic, v_dynamic, int(sample_gap), compensated_rows)
-        return res if out is None else out.copy_(res)
+        return res if out is None else autograd.copy_into(out, res)
     plan = ops.PLAN_CACHE.get(mask)
     out, _ = ops.block_sparse_attention_comp(q, k, v, plan, k_dynamic, v_dynamic, int(sample_gap),
                                              comp_rows=compensated_rows, return_lse=False, out=out)

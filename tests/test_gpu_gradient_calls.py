@@ -60,3 +60,19 @@ def test_pool_odd_strides(what, B, N):
     if what != "one row":
         more = odd_view(x, what)
         assert torch.equal(ops.mean_pool_tokens_backward(d, N, gap, add=more), ops.mean_pool_tokens_backward(d, N, gap, add=x))
+
+
+def test_compensation_into_a_buffer_used_again():
+    """The compensated call's `out` as a buffer that every step writes."""
+    N, gap = 400, 30
+    mask = make_mask(1, 2, N, N, 0.6, seed=74)
+    out = torch.empty(1, 2, N, 128, dtype=torch.bfloat16, device="cuda")
+    for seed in range(3):
+        q, k, v, do = make(1, 2, N, N, 128, torch.bfloat16, seed=80 + seed)
+        kd, vd = ops.mean_pool_kv(k, v, gap)
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        fresh = sa._block_sparse_attn_with_compensation(*leaves, mask, kd, vd, gap)
+        want = torch.autograd.grad(fresh, leaves, do)
+        got = sa._block_sparse_attn_with_compensation(*leaves, mask, kd, vd, gap, out=out)
+        assert got is out and torch.equal(got, fresh)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, leaves, do), want))

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from sinkattn_amd import ops
+from sinkattn_amd import autograd, ops
 
 
 def odd_views(dtype):
@@ -36,3 +36,43 @@ def test_operands_and_gradients_of_odd_strides(dtype, what):
 def test_gradients_keep_the_order_of_dims(layout):
     t = torch.zeros(2, 3, 40, 64) if layout == "bhnd" else torch.zeros(2, 40, 3, 64).transpose(1, 2)
     assert ops._grad_output(t, torch.float32).stride() == t.stride()
+
+
+class _Twice(torch.autograd.Function):
+    """A step whose saved tensors are gone after its backward pass."""
+
+    @staticmethod
+    def forward(ctx, x):
+        ctx.save_for_backward(x)
+        return 2 * x
+
+    @staticmethod
+    def backward(ctx, g):
+        return 2 * g + 0 * ctx.saved_tensors[0]
+
+
+def test_copy_into_a_buffer_used_again():
+    """A buffer that every call writes: no call's graph holds an earlier one's."""
+    x = torch.ones(2, 3, requires_grad=True)
+    out = torch.empty(2, 3)
+    for i in range(3):
+        assert autograd.copy_into(out, _Twice.apply(x)) is out
+        edges = out.grad_fn.next_functions
+        assert [e[0] for e in edges].count(None) == len(edges) - 1
+        (g,) = torch.autograd.grad(out.sum(), x)
+        assert torch.equal(g, torch.full((2, 3), 2.0))
+    # without a backward pass between the calls, and where something still reads the earlier result
+    first = autograd.copy_into(out, _Twice.apply(x)) * 3
+    autograd.copy_into(out, _Twice.apply(x))
+    assert torch.equal(torch.autograd.grad(first.sum(), x)[0], torch.full((2, 3), 6.0))
+    assert torch.equal(torch.autograd.grad(out.sum(), x)[0], torch.full((2, 3), 2.0))
+
+
+def test_copy_into_parts_of_a_buffer():
+    """Views of one buffer, written one after the other: each part's gradient arrives."""
+    x, y = (torch.ones(3, requires_grad=True) for _ in range(2))
+    base = torch.zeros(2, 3)
+    for i, t in enumerate((x, y)):
+        autograd.copy_into(base[i], _Twice.apply(t))
+    for g in torch.autograd.grad(base.sum(), (x, y)):
+        assert torch.equal(g, torch.full((3,), 2.0))
