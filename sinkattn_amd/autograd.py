@@ -31,19 +31,21 @@ def copy_into(out: torch.Tensor, res: torch.Tensor) -> torch.Tensor:
     return out.copy_(res)
 
 
-def _plans(mask: torch.Tensor) -> Tuple[ops.BlockSparsePlan, ops.BlockSparsePlan]:
-    """The mask's plan and key plan.  A capture makes both of its own, from the mask as it is at each replay: a
-    cached plan may be freed before the graph, and one made by a graph holds nothing before a replay."""
+def _plan(mask: torch.Tensor) -> ops.BlockSparsePlan:
+    """A plan of the mask as it is now, made on the current stream and kept by nothing but the call's graph: no write
+    to the mask, from wherever it comes, is missed.  Its launch order comes from the stream's cache of orders by tile
+    counts, but not in a capture, whose replays may run beside that stream."""
     with torch.cuda.device(mask.device):
-        if torch.cuda.is_current_stream_capturing():
-            return ops.block_sparse_plan(mask), ops.block_sparse_plan(mask.transpose(2, 3))
-    return ops.GRAD_PLAN_CACHE.get(mask)
+        captured = torch.cuda.is_current_stream_capturing()
+    if captured or mask.dim() != 4 or mask.numel() == 0:
+        return ops.block_sparse_plan(mask)
+    return ops.block_sparse_plan(mask, ops.PLAN_CACHE.order_cache(mask), ops.PLAN_CACHE.ORDER_CACHE_ENTRIES)
 
 
 class _BlockSparseAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, return_lse):
-        ctx.plan, ctx.key_plan = _plans(mask)
+        ctx.plan, ctx.key_plan = _plan(mask), _plan(mask.transpose(2, 3))
         out, lse = ops.block_sparse_attention(q, k, v, ctx.plan)
         ctx.save_for_backward(q, k, v, out, lse)
         ctx.set_materialize_grads(False)
@@ -72,7 +74,7 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ma
 class _BlockSparseAttentionComp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, kd, vd, mask, gap, comp_rows):
-        ctx.plan, ctx.key_plan = _plans(mask)
+        ctx.plan, ctx.key_plan = _plan(mask), _plan(mask.transpose(2, 3))
         ctx.gap, ctx.comp_rows = gap, comp_rows
         out, lse = ops.block_sparse_attention_comp(q, k, v, ctx.plan, kd, vd, gap, comp_rows=comp_rows, return_lse=True)
         ctx.save_for_backward(q, k, v, kd, vd, out, lse)
@@ -97,7 +99,7 @@ def block_sparse_attention_comp(q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
 class _BlockSparseAttentionPooled(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, gap, prefix, pool_end, comp_rows):
-        ctx.plan, ctx.key_plan = _plans(mask)
+        ctx.plan, ctx.key_plan = _plan(mask), _plan(mask.transpose(2, 3))
         ctx.pool, ctx.comp_rows = (gap, prefix, pool_end), comp_rows
         kd, vd = ops.mean_pool_kv(k, v, gap, prefix, pool_end)
         out, lse = ops.block_sparse_attention_comp(q, k, v, ctx.plan, kd, vd, gap, comp_rows=comp_rows, return_lse=True)

@@ -166,31 +166,6 @@ class _PlanCache:
 PLAN_CACHE = _PlanCache()
 
 
-class _GradPlanCache:
-    """The plan and the key plan (`block_sparse_plan` of the transposed mask) of a mask, keyed by its identity,
-    version and the stream that builds and uses them."""
-
-    def __init__(self) -> None:
-        self._entries: Dict[tuple, tuple] = {}
-
-    def get(self, mask: torch.Tensor) -> Tuple[BlockSparsePlan, BlockSparsePlan]:
-        key = (id(mask), torch.cuda.current_stream(mask.device).cuda_stream)
-        sig = (mask._version, mask.data_ptr(), tuple(mask.shape), tuple(mask.stride()), mask.device)
-        ent = self._entries.get(key)
-        if ent is not None and ent[0]() is mask and ent[1] == sig:
-            return ent[2]
-        plans = block_sparse_plan(mask), block_sparse_plan(mask.transpose(2, 3))
-        entries = self._entries
-        entries[key] = (weakref.ref(mask, lambda _r, k=key: entries.pop(k, None)), sig, plans)
-        return plans
-
-    def clear(self) -> None:
-        self._entries.clear()
-
-
-GRAD_PLAN_CACHE = _GradPlanCache()
-
-
 def _check_output(out: torch.Tensor, q: torch.Tensor) -> None:
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
         raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {q.device}, got {tuple(out.shape)} {out.dtype}")

@@ -643,7 +643,9 @@ def _block_sparse_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_
 
     q [B,H,Nq,D], k/v [B,H,Nk,D]; block_mask bool [B,H,ceil(Nq/128),ceil(Nk/128)].
     Returns out [B,H,Nq,D] (a view of [B,Nq,H,D] memory) and lse [B,H,Nq,1] in q.dtype
-    (or None), both differentiable.  The kernel's list form of the mask is cached per mask tensor.
+    (or None), both differentiable.  Without gradients the kernel's list form of the mask is cached per mask
+    tensor and version (a write that torch does not count, such as a replayed graph's, needs
+    `ops.PLAN_CACHE.clear()`); a differentiable call makes it from the mask as it is.
     """
     _ensure_block_sparse_available()
     mask = block_mask if block_mask.is_cuda else block_mask.to(q.device)

@@ -76,3 +76,84 @@ def test_compensation_into_a_buffer_used_again():
         got = sa._block_sparse_attn_with_compensation(*leaves, mask, kd, vd, gap, out=out)
         assert got is out and torch.equal(got, fresh)
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, leaves, do), want))
+
+
+def op_gradients(q, k, v, do, mask):
+    plan, kplan = plans(mask)
+    out, lse = ops.block_sparse_attention(q, k, v, plan)
+    return [out, *ops.block_sparse_attention_backward(do, q, k, v, out, lse, plan, kplan)]
+
+
+def call_gradients(leaves, do, mask):
+    out, _ = sa._block_sparse_attn(*leaves, mask)
+    return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+
+
+def same(a, b):
+    return len(a) == len(b) and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_mask_written_by_a_graph():
+    """A mask buffer that a replayed graph fills, which torch does not count as a change of the tensor: each call takes
+    the mask as it is."""
+    N, D = 700, 64
+    q, k, v, do = make(1, 2, N, N, D, torch.bfloat16, seed=75)
+    masks = [make_mask(1, 2, N, N, 0.5, seed=s) for s in (75, 76)]
+    want = [op_gradients(q, k, v, do, m) for m in masks]
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    source, mask = masks[0].clone(), torch.zeros_like(masks[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mask.copy_(source)
+    for turn in (0, 1, 1, 0):
+        source.copy_(masks[turn])
+        version = mask._version
+        graph.replay()
+        assert mask._version == version
+        for _ in range(2):
+            assert same(call_gradients(leaves, do, mask), want[turn])
+
+
+def test_mask_changed_before_the_backward_pass():
+    """The backward pass takes the mask that the forward saw."""
+    q, k, v, do = make(1, 2, 500, 600, 64, torch.float16, seed=77)
+    masks = [make_mask(1, 2, 500, 600, 0.5, seed=s) for s in (77, 78)]
+    want = op_gradients(q, k, v, do, masks[0])
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    mask = masks[0].clone()
+    out, _ = sa._block_sparse_attn(*leaves, mask)
+    mask.copy_(masks[1])
+    for _ in range(2):
+        assert same(torch.autograd.grad(out, leaves, do, retain_graph=True), want[1:])
+    del mask
+    assert same(torch.autograd.grad(out, leaves, do), want[1:])
+
+
+def test_mask_made_in_inference_mode():
+    q, k, v, do = make(1, 2, 300, 300, 64, torch.bfloat16, seed=79)
+    mask = make_mask(1, 2, 300, 300, 0.6, seed=79)
+    with torch.inference_mode():
+        kept = mask.clone()
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    assert same(call_gradients(leaves, do, kept), op_gradients(q, k, v, do, mask))
+
+
+def test_one_mask_on_two_streams():
+    """Differentiable calls on two streams at once that share one mask: the bits of calls one by one."""
+    N, D = 1500, 128
+    mask = make_mask(1, 3, N, N, 0.4, seed=81)
+    sets = [make(1, 3, N, N, D, torch.bfloat16, seed=81 + i) for i in range(2)]
+    want = [op_gradients(*s, mask) for s in sets]
+    leaves = [[t.clone().requires_grad_() for t in s[:3]] for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(3):
+        fresh = mask.clone()
+        got = []
+        for stream, ls, s in zip(streams, leaves, sets):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                got.append(call_gradients(ls, s[3], fresh))
+        torch.cuda.synchronize()
+        assert all(same(g, w) for g, w in zip(got, want))
