@@ -42,10 +42,27 @@ def _plan(mask: torch.Tensor) -> ops.BlockSparsePlan:
     return ops.block_sparse_plan(mask, ops.PLAN_CACHE.order_cache(mask), ops.PLAN_CACHE.ORDER_CACHE_ENTRIES)
 
 
+MAX_QUERY_BLOCKS = 8192  # of the transposed mask's plan
+
+
+def _plans(mask: torch.Tensor) -> Tuple[ops.BlockSparsePlan, Optional[ops.BlockSparsePlan]]:
+    """The mask's plan and key plan; no key plan where the mask has more query blocks than one takes: the forward
+    runs all the same, and a backward pass says so."""
+    plan = _plan(mask)
+    return plan, _plan(mask.transpose(2, 3)) if plan.shape[2] <= MAX_QUERY_BLOCKS else None
+
+
+def _key_plan(ctx) -> ops.BlockSparsePlan:
+    if ctx.key_plan is None:
+        raise RuntimeError(f"block-sparse attention gradient: {ctx.plan.shape[2]} blocks of queries, at most {MAX_QUERY_BLOCKS} "
+                           "are supported")
+    return ctx.key_plan
+
+
 class _BlockSparseAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, return_lse):
-        ctx.plan, ctx.key_plan = _plan(mask), _plan(mask.transpose(2, 3))
+        ctx.plan, ctx.key_plan = _plans(mask)
         out, lse = ops.block_sparse_attention(q, k, v, ctx.plan)
         ctx.save_for_backward(q, k, v, out, lse)
         ctx.set_materialize_grads(False)
@@ -61,7 +78,7 @@ class _BlockSparseAttention(torch.autograd.Function):
             dout = torch.zeros_like(out)
         if dlse is not None:
             dlse = dlse.squeeze(-1).float()
-        return (*ops.block_sparse_attention_backward(dout, q, k, v, out, lse, ctx.plan, ctx.key_plan, dlse=dlse),
+        return (*ops.block_sparse_attention_backward(dout, q, k, v, out, lse, ctx.plan, _key_plan(ctx), dlse=dlse),
                 None, None)
 
 
@@ -74,7 +91,7 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ma
 class _BlockSparseAttentionComp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, kd, vd, mask, gap, comp_rows):
-        ctx.plan, ctx.key_plan = _plan(mask), _plan(mask.transpose(2, 3))
+        ctx.plan, ctx.key_plan = _plans(mask)
         ctx.gap, ctx.comp_rows = gap, comp_rows
         out, lse = ops.block_sparse_attention_comp(q, k, v, ctx.plan, kd, vd, gap, comp_rows=comp_rows, return_lse=True)
         ctx.save_for_backward(q, k, v, kd, vd, out, lse)
@@ -84,7 +101,7 @@ class _BlockSparseAttentionComp(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, kd, vd, out, lse = ctx.saved_tensors
-        grads = ops.block_sparse_attention_comp_backward(dout, q, k, v, out, lse, ctx.plan, ctx.key_plan, kd, vd, ctx.gap,
+        grads = ops.block_sparse_attention_comp_backward(dout, q, k, v, out, lse, ctx.plan, _key_plan(ctx), kd, vd, ctx.gap,
                                                          comp_rows=ctx.comp_rows)
         return (*grads, None, None, None)
 
@@ -99,7 +116,7 @@ def block_sparse_attention_comp(q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
 class _BlockSparseAttentionPooled(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, gap, prefix, pool_end, comp_rows):
-        ctx.plan, ctx.key_plan = _plan(mask), _plan(mask.transpose(2, 3))
+        ctx.plan, ctx.key_plan = _plans(mask)
         ctx.pool, ctx.comp_rows = (gap, prefix, pool_end), comp_rows
         kd, vd = ops.mean_pool_kv(k, v, gap, prefix, pool_end)
         out, lse = ops.block_sparse_attention_comp(q, k, v, ctx.plan, kd, vd, gap, comp_rows=comp_rows, return_lse=True)
@@ -112,7 +129,7 @@ class _BlockSparseAttentionPooled(torch.autograd.Function):
         q, k, v, kd, vd, out, lse = ctx.saved_tensors
         gap, prefix, pool_end = ctx.pool
         dq, dk, dv, dkd, dvd = ops.block_sparse_attention_comp_backward(
-            dout, q, k, v, out, lse, ctx.plan, ctx.key_plan, kd, vd, gap, comp_rows=ctx.comp_rows,
+            dout, q, k, v, out, lse, ctx.plan, _key_plan(ctx), kd, vd, gap, comp_rows=ctx.comp_rows,
             key_grad_dtype=torch.float32)
         # the pooled keys' share joins the attention's in fp32: one rounding of the whole gradient
         dk, dv = ops.mean_pool_kv_backward(dkd, dvd, int(k.shape[2]), gap, prefix, pool_end, add=(dk, dv), out_dtype=k.dtype)

@@ -157,3 +157,25 @@ def test_one_mask_on_two_streams():
                 got.append(call_gradients(ls, s[3], fresh))
         torch.cuda.synchronize()
         assert all(same(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.parametrize("comp", [False, True])
+def test_more_query_blocks_than_a_key_plan_takes(comp):
+    """Such calls run where an input asks for a gradient, with the results of a call without; their backward passes raise."""
+    N, D, gap = 8192 * 128 + 5, 128 if comp else 32, 30
+    g = torch.Generator(device="cuda").manual_seed(86)
+    q, k, v = (torch.randn(1, 1, n, D, device="cuda", generator=g).bfloat16() for n in (N, 200, 200))
+    mask = torch.ones(1, 1, 8193, 2, dtype=torch.bool, device="cuda")
+    kd, vd = ops.mean_pool_kv(k, v, gap)
+
+    def call(q, k, v):
+        if comp:
+            return sa._block_sparse_attn_with_compensation(q, k, v, mask, kd, vd, gap)
+        return sa._block_sparse_attn(q, k, v, mask)[0]
+
+    plain = call(q, k, v)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = call(*leaves)
+    assert torch.equal(out, plain)
+    with pytest.raises(RuntimeError, match="8193 blocks of queries"):
+        torch.autograd.grad(out, leaves, torch.zeros_like(out))
