@@ -5,21 +5,30 @@ recorded and an input asks for one; without gradients they call `ops` directly. 
 are the same bits either way.  What a forward saves is what torch's own attention saves: its
 operands, its output and the fp32 log-sum-exp; probabilities are recomputed in the backward pass,
 which runs on the forward's stream, allocates through torch and can be captured into a graph with it.
-Second derivatives are refused.
+Second derivatives and forward-mode differentiation are refused.
 """
 from __future__ import annotations
 
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
 
 
+def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether one of the tensors carries a tangent of forward-mode differentiation."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # outside every dual level
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def needs_grad(*tensors: Optional[torch.Tensor]) -> bool:
-    """Whether gradients are recorded and one of the tensors asks for one."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether gradients are recorded and one of the tensors asks for one, or one carries a tangent (which the forms
+    below refuse, and a kernel's plain call would drop)."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or has_tangent(*tensors)
 
 
 def copy_into(out: torch.Tensor, res: torch.Tensor) -> torch.Tensor:

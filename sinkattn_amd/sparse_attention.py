@@ -104,8 +104,9 @@ def _pad_to_multiple(x: torch.Tensor, multiple: int) -> torch.Tensor:
 
 
 def _token_pool_on_gpu(x: torch.Tensor) -> bool:
-    """GPU tensors go to the mean_pool_tokens kernel; host tensors keep the torch ops."""
-    return x.is_cuda and x.dim() == 4
+    """GPU tensors go to the mean_pool_tokens kernel; host tensors, and those with a forward-mode tangent, keep the
+    torch ops."""
+    return x.is_cuda and x.dim() == 4 and not autograd.has_tangent(x)
 
 
 def _mean_pool_sequence(x: torch.Tensor, pool_size: int) -> torch.Tensor:

@@ -326,8 +326,8 @@ def _fused_qk_prep(attn, query: torch.Tensor, key: torch.Tensor, rotary_emb):
         if tables is None or tables[0].size(0) != int(query.size(1)):
             return None
     fr, fi = tables if tables is not None else (None, None)
-    if autograd.needs_grad(fr, fi):
-        return None  # the kernel's tables are constants
+    if autograd.needs_grad(fr, fi) or autograd.has_tangent(query, key, pq[0], pk[0]):
+        return None  # the kernel's tables are constants, and it carries no forward-mode tangents
     prep = autograd.qk_norm_rotary if autograd.needs_grad(query, key, pq[0], pk[0]) else ops.qk_norm_rotary
     return prep(query, key, pq[0], pk[0], pq[1], pk[1], D, fr, fi, rows_per_pos=1)
 

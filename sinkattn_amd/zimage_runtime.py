@@ -235,8 +235,8 @@ def _fused_qk_prep(attn: Any, q: torch.Tensor, k: torch.Tensor, freqs_cis: Optio
         if f.size(0) not in (N, B * N):
             return None
         fr, fi = f.real, f.imag
-    if autograd.needs_grad(fr, fi):
-        return None  # the kernel's tables are constants
+    if autograd.needs_grad(fr, fi) or autograd.has_tangent(q, k, pq[0], pk[0]):
+        return None  # the kernel's tables are constants, and it carries no forward-mode tangents
     prep = autograd.qk_norm_rotary if autograd.needs_grad(q, k, pq[0], pk[0]) else ops.qk_norm_rotary
     return prep(q, k, pq[0], pk[0], pq[1], pk[1], D, fr, fi, rows_per_pos=int(q.size(2)))
 

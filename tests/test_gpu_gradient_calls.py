@@ -1,14 +1,14 @@
 """Calls of the gradient operators and their autograd forms that a program may make around the usual ones: operands of
 unusual strides, buffers used again, masks that change, streams, other ways of differentiation."""
-import math
-
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from sinkattn_amd import autograd, ops
+from sinkattn_amd import ops
 from sinkattn_amd import sparse_attention as sa
+from sinkattn_amd import wan_runtime as wr
 
-from backward_bars import check, formula, make, make_mask, plans
+from backward_bars import make, make_mask, plans
 
 pytestmark = pytest.mark.gpu
 
@@ -179,3 +179,41 @@ def test_more_query_blocks_than_a_key_plan_takes(comp):
     assert torch.equal(out, plain)
     with pytest.raises(RuntimeError, match="8193 blocks of queries"):
         torch.autograd.grad(out, leaves, torch.zeros_like(out))
+
+
+def test_forward_mode():
+    """The attention refuses tangents instead of dropping them; pooling and QK norms carry them."""
+    N, gap = 260, 30
+    q, k, v, t = make(1, 2, N, N, 128, torch.bfloat16, layout="bhnd", seed=87)
+    mask = make_mask(1, 2, N, N, 1.0)
+    kd, vd = ops.mean_pool_kv(k, v, gap)
+    with forward_ad.dual_level():
+        for i in range(3):
+            args = [q, k, v]
+            args[i] = forward_ad.make_dual(args[i], t)
+            for grad in (torch.enable_grad, torch.no_grad):
+                with grad():
+                    with pytest.raises(NotImplementedError):
+                        sa._block_sparse_attn(*args, mask)
+                    with pytest.raises(NotImplementedError):
+                        sa._block_sparse_attn_with_compensation(*args, mask, kd, vd, gap)
+                    with pytest.raises(NotImplementedError):
+                        wr.WanSinkSparseInnerAttention(0, mask[0], sa.SinkSparseConfig(sample_gap=gap))(*args)
+        x = forward_ad.make_dual(k, t)
+        for prefix in (0, 17):
+            y = sa._mean_pool_sequence_preserve_prefix(x, gap, prefix_tokens=prefix)
+            tangent = forward_ad.unpack_dual(y).tangent
+            # the pooling is linear: the tangent is the pooled tangent, a sum of `gap` terms and two roundings apart
+            # from the kernel's
+            want = ops.mean_pool_tokens(t, gap, prefix).double()
+            bound = 2 * torch.finfo(t.dtype).eps * ops.mean_pool_tokens(t.abs(), gap, prefix).double() * 1.05
+            assert ((tangent.double() - want).abs() <= bound).all()
+
+    class Norms:
+        heads = 2
+        norm_q, norm_k = (torch.nn.RMSNorm(256, eps=1e-6, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+
+    rows = [u.transpose(1, 2).flatten(2) for u in (q, k, t)]
+    assert wr._fused_qk_prep(Norms, rows[0], rows[1], None) is not None
+    with forward_ad.dual_level():
+        assert wr._fused_qk_prep(Norms, forward_ad.make_dual(rows[0], rows[2]), rows[1], None) is None

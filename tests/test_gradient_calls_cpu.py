@@ -1,6 +1,7 @@
 """What the gradient operators and their autograd forms do around a launch, as far as it needs no GPU."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from sinkattn_amd import autograd, ops
 
@@ -76,3 +77,15 @@ def test_copy_into_parts_of_a_buffer():
         autograd.copy_into(base[i], _Twice.apply(t))
     for g in torch.autograd.grad(base.sum(), (x, y)):
         assert torch.equal(g, torch.full((3,), 2.0))
+
+
+def test_tangents_are_seen():
+    x = torch.ones(1, 1, 8, 64)
+    assert not autograd.has_tangent(x, None)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, x)
+        assert autograd.has_tangent(None, d) and autograd.needs_grad(x, d)
+        assert not autograd.has_tangent(x, torch.zeros(2, dtype=torch.bool)) and not autograd.needs_grad(x)
+        with torch.no_grad():
+            assert autograd.needs_grad(d)  # forward mode goes on without recorded gradients
+    assert not autograd.needs_grad(x)
