@@ -124,10 +124,9 @@ def block_sparse_attention_comp(q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
 
 class _BlockSparseAttentionPooled(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, mask, gap, prefix, pool_end, comp_rows):
+    def forward(ctx, q, k, v, kd, vd, mask, gap, prefix, pool_end, comp_rows):
         ctx.plan, ctx.key_plan = _plans(mask)
         ctx.pool, ctx.comp_rows = (gap, prefix, pool_end), comp_rows
-        kd, vd = ops.mean_pool_kv(k, v, gap, prefix, pool_end)
         out, lse = ops.block_sparse_attention_comp(q, k, v, ctx.plan, kd, vd, gap, comp_rows=comp_rows, return_lse=True)
         ctx.save_for_backward(q, k, v, kd, vd, out, lse)
         return out
@@ -142,15 +141,17 @@ class _BlockSparseAttentionPooled(torch.autograd.Function):
             key_grad_dtype=torch.float32)
         # the pooled keys' share joins the attention's in fp32: one rounding of the whole gradient
         dk, dv = ops.mean_pool_kv_backward(dkd, dvd, int(k.shape[2]), gap, prefix, pool_end, add=(dk, dv), out_dtype=k.dtype)
-        return dq, dk, dv, None, None, None, None, None
+        return dq, dk, dv, None, None, None, None, None, None, None
 
 
 def block_sparse_attention_pooled(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: torch.Tensor, gap: int,
                                   prefix: int = 0, pool_end: Optional[int] = None,
-                                  comp_rows: Optional[int] = None) -> torch.Tensor:
+                                  comp_rows: Optional[int] = None,
+                                  pooled: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> torch.Tensor:
     """`ops.mean_pool_kv` and the compensated attention over its rows as one step of the graph, so that K
-    and V get one gradient each."""
-    return _BlockSparseAttentionPooled.apply(q, k, v, mask, gap, prefix, pool_end, comp_rows)
+    and V get one gradient each.  `pooled`: that call's rows of these K and V, where the caller has made them."""
+    kd, vd = ops.mean_pool_kv(k, v, gap, prefix, pool_end) if pooled is None else pooled
+    return _BlockSparseAttentionPooled.apply(q, k, v, kd, vd, mask, gap, prefix, pool_end, comp_rows)
 
 
 class _MeanPoolTokens(torch.autograd.Function):

@@ -183,16 +183,13 @@ class WanSinkSparseInnerAttention(nn.Module):
             elif (self.config.mixing_mode == "adaptive" and FUSE_COMPENSATION
                   and _fused_compensation_supported(q, k, v)):
                 prefix = max(int(self.config.text_length), 0)
-                if autograd.needs_grad(q, k, v):
-                    first = min(prefix, int(k.size(2)))
-                    dyn_len = first + _ceil_div(int(k.size(2)) - first, gap)
-                    with _section(rs, "sparse_main"):  # pooling + sparse + compensation + mix
-                        out = autograd.block_sparse_attention_pooled(q, k, v, mask, gap, prefix)
-                else:
-                    with _section(rs, "comp_pool"):
-                        k_dyn, v_dyn = ops.mean_pool_kv(k, v, gap, prefix)
-                        dyn_len = int(k_dyn.size(2))
-                    with _section(rs, "sparse_main"):  # sparse + compensation + mix
+                with _section(rs, "comp_pool"):
+                    k_dyn, v_dyn = ops.mean_pool_kv(k, v, gap, prefix)
+                    dyn_len = int(k_dyn.size(2))
+                with _section(rs, "sparse_main"):  # sparse + compensation + mix
+                    if autograd.needs_grad(q, k, v):
+                        out = autograd.block_sparse_attention_pooled(q, k, v, mask, gap, prefix, pooled=(k_dyn, v_dyn))
+                    else:
                         out = _block_sparse_attn_with_compensation(q, k, v, mask, k_dyn, v_dyn, gap)
             else:
                 adaptive = self.config.mixing_mode == "adaptive"

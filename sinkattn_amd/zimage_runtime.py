@@ -549,17 +549,15 @@ class ZImageStaticSinkProcessor:
                 elif (mode == "pooled_kv" and FUSE_COMPENSATION and self.image_token_count % 128 == 0
                       and _fused_compensation_supported(q_i, k_i, v_i)):
                     il = self.image_token_count
-                    if grad:
-                        dyn_len = _ceil_div(il, gap) + n - il
-                        with sec("sparse_main"):  # pooling + sparse + compensation on the image rows + mix
+                    with sec("comp_pool"):
+                        # the pooled image keys, then the text keys
+                        dyn_k, dyn_v = ops.mean_pool_kv(k_i, v_i, gap, pool_end=il)
+                        dyn_len = int(dyn_k.size(2))
+                    with sec("sparse_main"):  # sparse + compensation on the image rows + mix
+                        if grad:
                             out_i = autograd.block_sparse_attention_pooled(q_i, k_i, v_i, mask, gap, pool_end=il,
-                                                                           comp_rows=il)
-                    else:
-                        with sec("comp_pool"):
-                            # the pooled image keys, then the text keys
-                            dyn_k, dyn_v = ops.mean_pool_kv(k_i, v_i, gap, pool_end=il)
-                            dyn_len = int(dyn_k.size(2))
-                        with sec("sparse_main"):  # sparse + compensation on the image rows + mix
+                                                                           comp_rows=il, pooled=(dyn_k, dyn_v))
+                        else:
                             out_i = _block_sparse_attn_with_compensation(q_i, k_i, v_i, mask, dyn_k, dyn_v, gap,
                                                                          compensated_rows=il, out=into)
                     run_mode = mode

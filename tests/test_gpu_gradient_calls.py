@@ -6,7 +6,9 @@ from torch.autograd import forward_ad
 
 from sinkattn_amd import ops
 from sinkattn_amd import sparse_attention as sa
+from sinkattn_amd import timing
 from sinkattn_amd import wan_runtime as wr
+from sinkattn_amd import zimage_runtime as zr
 
 from backward_bars import make, make_mask, plans
 
@@ -217,3 +219,55 @@ def test_forward_mode():
     assert wr._fused_qk_prep(Norms, rows[0], rows[1], None) is not None
     with forward_ad.dual_level():
         assert wr._fused_qk_prep(Norms, forward_ad.make_dual(rows[0], rows[2]), rows[1], None) is None
+
+
+def timed():
+    state = sa.SinkRuntimeState()
+    state.timing = timing.AttentionTimingCollector(label="sink", enabled=True)
+    return state
+
+
+def sections(state):
+    return {name: entry["count"] for name, entry in state.summarize_timing()["by_section"].items()}
+
+
+def test_timing_sections_with_gradients():
+    """A layer call records the same sections and pooled lengths whether an input asks for a gradient or not."""
+    N, text = 700, 40
+    q, k, v, _ = make(1, 2, N, N, 128, torch.bfloat16, seed=88)
+    mask = make_mask(1, 2, N, N, 0.5, seed=88)
+    seen = []
+    for grad in (False, True):
+        state = timed()
+        layer = wr.WanSinkSparseInnerAttention(0, mask[0], sa.SinkSparseConfig(sample_gap=30, text_length=text), runtime_state=state)
+        layer(*(t.clone().requires_grad_(grad) for t in (q, k, v)))
+        seen.append((sections(state), state.sparsity_events))
+    assert "comp_pool" in seen[0][0] and seen[0] == seen[1]
+
+
+def test_timing_sections_of_an_image_layer_with_gradients():
+    H, D, side, text = 2, 128, 16, 20
+    cfg = zr.build_zimg_sink_config(config_overrides=dict(token_width=side, token_height=side, dynamic_mode="pooled_kv",
+                                                          sample_gap=30))
+    nb = zr._fixed_block_shape(cfg)[2]
+
+    class Layer(torch.nn.Module):
+        heads = H
+
+        def __init__(self):
+            super().__init__()
+            self.to_q, self.to_k, self.to_v = (torch.nn.Linear(H * D, H * D) for _ in range(3))
+            self.to_out = torch.nn.ModuleList([torch.nn.Linear(H * D, H * D)])
+            self.norm_q, self.norm_k = (torch.nn.RMSNorm(D, eps=1e-6) for _ in range(2))
+
+    layer = Layer().bfloat16().cuda()
+    x = torch.randn(1, side * side + text, H * D, device="cuda").bfloat16()
+    seen = []
+    for grad in (False, True):
+        state = timed()
+        proc = zr.ZImageStaticSinkProcessor(layer_idx=0, total_layers=2, sink_mask=torch.ones(H, nb, nb, dtype=torch.bool),
+                                            config=cfg, runtime_state=state)
+        with torch.set_grad_enabled(grad):
+            proc(layer, x)
+        seen.append((sections(state), state.sparsity_events))
+    assert "comp_pool" in seen[0][0] and seen[0] == seen[1]
