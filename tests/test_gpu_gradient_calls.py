@@ -1,5 +1,7 @@
 """Calls of the gradient operators and their autograd forms that a program may make around the usual ones: operands of
 unusual strides, buffers used again, masks that change, streams, other ways of differentiation."""
+import math
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -10,7 +12,7 @@ from sinkattn_amd import timing
 from sinkattn_amd import wan_runtime as wr
 from sinkattn_amd import zimage_runtime as zr
 
-from backward_bars import make, make_mask, plans
+from backward_bars import check, formula, make, make_mask, plans
 
 pytestmark = pytest.mark.gpu
 
@@ -271,3 +273,35 @@ def test_timing_sections_of_an_image_layer_with_gradients():
             proc(layer, x)
         seen.append((sections(state), state.sparsity_events))
     assert "comp_pool" in seen[0][0] and seen[0] == seen[1]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_more_heads_than_launch_chunks(dtype):
+    """More heads than a plan deals to the XCDs in chunks (4096): the launch order without a chunk table."""
+    B, H, N, D = 65, 64, 200, 32
+    q, k, v, do = make(B, H, N, N, D, dtype, seed=89)
+    mask = make_mask(B, H, N, N, 0.7, seed=89)
+    plan, kplan = plans(mask)
+    out, lse = ops.block_sparse_attention(q, k, v, plan)
+    grads = ops.block_sparse_attention_backward(do, q, k, v, out, lse, plan, kplan)
+    for b in (0, 31, 64):
+        at = slice(b, b + 1)
+        want, off = formula(q[at], k[at], v[at], do[at], out[at], lse[at], mask[at], 1 / math.sqrt(D))
+        check([g[at] for g in grads], want, off)
+    assert all(torch.isfinite(g).all() for g in grads)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,H,N", [(1, 1, 5000), (1, 6, 3300)])
+def test_long_lists_of_head_dim_32(dtype, B, H, N):
+    """Lists that are cut into parts at the smallest head dim."""
+    q, k, v, do = make(B, H, N, N, 32, dtype, seed=90)
+    mask = make_mask(B, H, N, N, 0.05, seed=90)
+    mask[..., 0] = mask[..., 17] = True
+    mask[:, :, 3] = True
+    plan, kplan = plans(mask)
+    out, lse = ops.block_sparse_attention(q, k, v, plan)
+    grads = ops.block_sparse_attention_backward(do, q, k, v, out, lse, plan, kplan)
+    want, off = formula(q, k, v, do, out, lse, mask, 1 / math.sqrt(32))
+    check(grads, want, off)
+    assert same(grads, ops.block_sparse_attention_backward(do, q, k, v, out, lse, plan, kplan))
