@@ -1009,11 +1009,13 @@ template <int CT>
 static hipError_t launch_bwd_dt(const BwdArgs& args, int D, hipStream_t stream) {
   BwdArgs a = args;
   const int nbh = a.B * a.H;
-  // The orders keep a head's blocks on one XCD, for its L2, which can leave the XCDs with unlike work where blocks are few (20%
-  // at 12 heads of 32).  fp32 products take so long that the reads matter less: there dQ 1.06 -> 0.94 ms in plain order.
-  // (24 heads of 64 blocks, uniform: 4.45 ms in the plan's order, 4.85 in plain.)
-  if (CT == kF32 && nbh * a.nqb < f32_round_blocks(D)) a.order = nullptr;
-  if (CT == kF32 && nbh * a.nkb < f32_round_blocks(D)) a.korder = nullptr;
+  // The orders keep a head's blocks on one XCD, for its L2, which leaves the XCDs with unlike work where heads are few and
+  // unlike.  fp32 products take so long that the reads matter less: with fewer than two heads for an XCD the plain order is
+  // faster (heads of densities of their own, whole calls in us, plan's -> plain order, D = 128: [1,8,4096] 1109 -> 1053,
+  // [1,10,4096] 1055 -> 955, [1,12,4096] 1529 -> 1471, [1,4,9000] 1764 -> 1627, [1,12,17000] 9042 -> 8480, [1,8,30000] 15002 ->
+  // 10440; the same at D = 64 and 32; six heads of 4096 lose 1%), with more the plan's (plain -> plan's: [1,16,4096] 1661 -> 1631,
+  // [1,18,4096] 1861 -> 1789, [1,32,4096] 4000 -> 3620, [1,24,7680] 4483 -> 4357, D = 64 [1,20,4096] 1117 -> 1066).
+  if (CT == kF32 && nbh < 2 * kXcds) a.order = a.korder = nullptr;
   const int qgrid = a.order ? plan_launch_slots(nbh * a.nqb, a.nqb) : nbh * a.nqb;
   const int kgrid = a.korder ? plan_launch_slots(nbh * a.nkb, a.nkb) : nbh * a.nkb;
   if (D == 128) return launch_bwd_d<CT, 128>(a, qgrid, kgrid, stream);
