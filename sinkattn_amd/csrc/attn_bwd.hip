@@ -15,8 +15,9 @@
 // The accumulators of the first two products hold a column per lane and the streamed rows in the
 // registers, which is the B operand of the others, so P and dS never leave the registers.  S and dP
 // are computed by both kernels (seven products in place of five): every gradient is then summed
-// by one group in a fixed order, without atomics, and results do not change from run to run.  (dS kept
-// for a second pass, five products in all, would cost 64 KB of traffic a tile: as much time as two products.)
+// by one group in a fixed order, without atomics, and results do not change from run to run.  (Five products in all would
+// need dS kept between them.  By arithmetic, not tried: 16-bit dS is 64 KB of traffic a tile, 13 ns of the chip's memory
+// against 7 ns for two products; in fp32 it is 128 KB, 26 ns against 54, so there it could pay.)
 // What bounds it, bf16, D = 128, 12 heads of 32760 tokens with 20% of the tiles: the power limit.  dQ takes 1.56 ms
 // (1.23 PFLOP/s of its three products), dK/dV 2.17 ms (1.18 of its four), at 1.72-1.76 GHz of 2.4 with the matrix cores
 // busy 63-66% of the cycles, on a card whose library product of 8192^3 reaches 1.13 PFLOP/s.  Short lists (24 heads
@@ -321,9 +322,11 @@ __device__ __forceinline__ int q_item_parts(const BwdArgs& a, int item) {
 // lists, and for the pooled keys.)  There are at most twice as many parts as shares, which k_slots allows for.
 // Where whole lists all run at once, a larger share may be the better one: a part costs its sums' way through memory
 // (of all parts together, about 60 ns each), a tile more on the longest list about kTileParts as much, and parts that do
-// not all run at once a second round.  30 heads of 9 blocks with four tiles each, D = 128: 31 us and 18 of the join with
-// shares of three, 27 and 4 with whole lists; with 2.3 tiles and 30 pooled blocks of eight: 38 and 18 with shares of two,
-// 37 and 14 with three, 50 and 9 with four and more (kTileParts = 24).
+// not all run at once a second round.  Whole calls with this choice of share against the even share, D = 128: [1,40,1101]
+// 88 against 104 us, [1,12,4000] 141 and 161, [2,12,2500] 143 and 162, [1,30,1101] with pooled keys 84 and 89, equal
+// at [1,12,2048] and [1,1,16000], and 54 against 53 at [1,8,2000,64].  kTileParts = 96 against 24 and 384: [1,24,1000] 62, 65 and
+// 66; [1,40,1101] 88, 96 and 88; [1,30,1101] with pooled keys 84, 92 and 84; [1,1,16000] 105, 117 and 105; [1,4,8190] with pooled keys
+// 154, 165 and 154; [1,12,5000] with them 214, 204 and 215; [1,16,2500,32] 60, 60 and 64.
 constexpr int kTileParts = 96;
 
 __device__ void plan_key_parts(const BwdArgs& a) {
@@ -462,7 +465,9 @@ __device__ __forceinline__ BwdItem bwd_item(const BwdArgs& a, int blk, int slots
     }
     blk -= kXcds;
     // A slot's parts follow each other.  Where all run at once, the first parts of all slots come first: of parts in turn, those
-    // without work would leave their neighbours two to a CU and other CUs idle (19 -> 24 us for 270 lists of one tile).
+    // without work would leave their neighbours two to a CU and other CUs idle (19 -> 24 us for 270 lists of one tile; whole calls
+    // in turn instead: [1,30,1101] with pooled keys 84 -> 92 us, [1,24,700] with them 60 -> 66, [1,16,2500,32] 60 -> 64, but
+    // [1,12,4000] 141 -> 138 and [1,1,16000] 105 -> 103).
     const int rounded = (slots + kXcds - 1) / kXcds * kXcds;
     const bool first_ones = a.k_one_round && rounded * a.q_parts <= 2 * a.k_shares;
     w.part = first_ones ? blk / rounded : blk / kXcds % a.q_parts;
@@ -947,7 +952,9 @@ size_t block_sparse_bwd_workspace(BwdArgs& a, int dtype, int D, void* workspace)
   const int64_t groups = (D == 128 ? 2 : D == 64 && dtype != kF32 ? 3 : 4) * device_cu_count();
   const int64_t qlist = a.nkb + ndb > 1 ? a.nkb + ndb : 1;
   // 16-bit: as many parts as run at once, or barely do not.  Where every list's blocks would not as parts of their own, parts
-  // have four blocks if lists allow (30 heads of 9 q-blocks with 2.3 tiles each and one of pooled keys: 44 -> 35 us).
+  // have four blocks if lists allow (30 heads of 9 q-blocks with 2.3 tiles each and one of pooled keys: 44 -> 35 us; whole calls
+  // with at most one, two, four and eight: [1,24,1000] 70, 63, 62 and 62 us, [1,40,1101] 95, 93, 88 and 85, [1,12,2048] 85,
+  // 85, 80 and 84, [1,4,8000] 119, 119, 117 and 109, [1,12,2000] with pooled keys 81, 79, 76 and 79).
   // fp32 (a block is two groups, and its blocks' products outweigh a part's sums by far): some rounds, for an even end.
   int64_t q_parts = rows > 0 && rows < groups ? (groups + rows - 1) / rows : 1;
   const int64_t dense_share = (rows * qlist + groups - 1) / groups;
