@@ -18,10 +18,11 @@
 // by one group in a fixed order, without atomics, and results do not change from run to run.  (Five products in all would
 // need dS kept between them.  By arithmetic, not tried: 16-bit dS is 64 KB of traffic a tile, 13 ns of the chip's memory
 // against 7 ns for two products; in fp32 it is 128 KB, 26 ns against 54, so there it could pay.)
-// What bounds it, bf16, D = 128, 12 heads of 32760 tokens with 20% of the tiles: the power limit.  dQ takes 1.56 ms
-// (1.23 PFLOP/s of its three products), dK/dV 2.17 ms (1.18 of its four), at 1.72-1.76 GHz of 2.4 with the matrix cores
-// busy 63-66% of the cycles, on a card whose library product of 8192^3 reaches 1.13 PFLOP/s.  Short lists (24 heads
-// of 8190 tokens: 0.35 + 0.44 ms, 0.85 PFLOP/s) pay some 17 us per round of work-groups for the columns' operands and results.
+// What bounds it, bf16, D = 128, 12 heads of 32760 tokens with 20% of the tiles: the power limit.  dQ takes 1.44 ms
+// (1.33 PFLOP/s of its three products), dK/dV 2.04 ms (1.26 of its four) on a card whose library product of 8192^3 reaches
+// 1.19 PFLOP/s, 1.56 and 2.17 ms on one with 1.13, there at 1.72-1.76 GHz of 2.4 with the matrix cores busy 63-66% of the
+// cycles.  f16 takes 1.65 + 2.32 ms on the first (library 1.18).  Short lists (24 heads of 8190 tokens with pooled keys: 0.31 + 0.39
+// ms, 1.18 PFLOP/s) pay some 17 us per round of work-groups for the columns' operands and results.
 // The dQ kernel runs first and leaves each row's lse (in log2 units) and -delta in the workspace.
 
 #include "common.h"
@@ -57,7 +58,7 @@ __device__ __forceinline__ Rows head_rows(const void* p, const int64_t (&s)[4], 
 // 32 columns a wave, because one wave per SIMD with 64 (half the LDS reads per product) had its accumulators in the
 // other half of the register file, with a move around every product: 2.8 ms for dK/dV above, 2.1 as it is.  D = 64 runs
 // three waves per SIMD and is bound by VALU work, an exponential and some six other instructions per 256 flops (2 x 16
-// heads of 8100 tokens, 25%, fp16: 0.25 + 0.32 ms, 0.86 PFLOP/s).
+// heads of 8100 tokens, 25%, fp16: 0.21 + 0.29 ms, 0.93 PFLOP/s; bf16 0.19 + 0.24; D = 32 0.15 + 0.19 and 0.13 + 0.15).
 // ------------------------------------------------------------------------------------
 constexpr float kPShift = 14.f;        // log2; P is at most 1, or barely above by the lse's rounding
 constexpr float kDsStart = 30.f;       // log2 of a column's first dS factor
@@ -757,8 +758,8 @@ __global__ __launch_bounds__(256) void attn_bwd_join_kernel(BwdArgs a) {
 // d = 16 c + 4 g + e of lane group g, four steps per 16-byte read; step i of the other products takes
 // streamed row 4 g + i, the row of accumulator register i, one 4-byte read per 16 columns d.  Chunks
 // are swizzled by row & 7: neither read has bank conflicts.  Bound by the matrix cores, busy 93%
-// of the time that a CU has work: 12 heads of 4096 tokens, 74%, D = 128 take 0.93 + 1.27 ms, 0.12 PFLOP/s of the seven
-// products where the library's 8192^3 reaches 0.154; the rest is the uneven end of lists of 12 to 32 tiles.
+// of the time that a CU has work: 12 heads of 4096 tokens, 74%, D = 128 take 0.93 + 1.27 ms, 0.13 PFLOP/s of the seven
+// products where the library's 8192^3 reaches 0.153 (D = 64 0.49 + 0.59, D = 32 0.27 + 0.30); the rest is the uneven end of lists of 12 to 32 tiles.
 // ------------------------------------------------------------------------------------
 template <int D, bool KEYS>
 __global__ __launch_bounds__(256, KEYS ? 2 : 3) void attn_bwd_f32_kernel(BwdArgs a, int slots) {
