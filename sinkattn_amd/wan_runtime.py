@@ -70,7 +70,7 @@ class WanSinkSparseInnerAttention(nn.Module):
     q, k, v are `[B, H, N, d]`.  The layer's mask `[H, nqb, nkb]` is widened once per
     (device, shape) to `mask | required | band` and expanded to the batch; the result
     is cached, so the kernel plan built from it is cached too (the plan cache keys on the
-    mask tensor)."""
+    mask tensor; calls with gradients build theirs anew)."""
 
     def __init__(self, layer_idx: int, sink_mask: torch.Tensor, config: SinkSparseConfig,
                  runtime_state: Optional[SinkRuntimeState] = None):
